@@ -14,7 +14,7 @@ OBJ=/tmp/hark_ab_$NAME; mkdir -p $OBJ
 EXCL=""
 for u in $UNITS; do
   base=$(basename $u)
-  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -munsafe-fp-atomics -Wno-unused-function -Wno-unused-value -Wno-unused-result -I. -I../../include $FLAGS -c $u -o $OBJ/${base%.hip}.o
+  /opt/rocm/bin/hipcc -O3 -std=c++17 -fPIC --offload-arch=gfx950 -munsafe-fp-atomics -Xclang -target-feature -Xclang -packed-fp32-ops -Wno-unused-function -Wno-unused-value -Wno-unused-result -I. -I../../include $FLAGS -c $u -o $OBJ/${base%.hip}.o
   EXCL="$EXCL ${base%.hip}.o"
 done
 OTHERS=$(ls *.o | grep -v -x -F "$(echo $EXCL | tr ' ' '\n')")
